@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(THREADS) block_tables_kernel(const __grid_cons
         run[0] += a;
         run[1] += pages_of(h + a, p.page) - pages_of(h, p.page);
     }
-    if (r0 < p.n && r1 == p.n) {
+    if (tid == THREADS - 1) {  // has all requests before it or its own, none if there are none
         starts[p.n] = saturate(run[0]);
         firsts[p.n] = saturate(run[1]);
     }

@@ -1,0 +1,62 @@
+"""The token-step operators where sizes, lengths and values run out: empty batches, bad lengths, the ends of number ranges."""
+import numpy as np
+import pytest
+
+import tadma_b200 as tb
+from tadma_b200.abi import Status
+from tests import token_step_reference as ref
+from tests.token_step_reference import UNIT, f64
+
+pytestmark = pytest.mark.gpu
+
+INDEX = 1 << Status.ERR_INDEX
+
+
+def torch_():
+    import torch
+    return torch
+
+
+def gen(seed):
+    return torch_().Generator(device="cuda").manual_seed(seed)
+
+
+def ints(v, dtype="int32"):
+    torch = torch_()
+    return torch.tensor(np.asarray(v), dtype=getattr(torch, dtype), device="cuda")
+
+
+@pytest.fixture(autouse=True)
+def _clean_flags():
+    tb.error_flags()
+    yield
+    tb.error_flags()
+
+
+# ------------------------------------------------------------ block tables --
+
+@pytest.mark.parametrize("slots_type", ["int32", "int64"])
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("cap", [0, 5, 3000])
+def test_block_tables_of_an_empty_batch(slots_type, strided, cap):
+    torch = torch_()
+    step = 3 if strided else 1
+
+    def out(n, dtype="int32"):
+        return torch.full((n * step,), 99, dtype=getattr(torch, dtype), device="cuda")[::step]
+
+    def call(held, added, left_in, slots, width):
+        n = len(held)
+        table = torch.full((n, width), -1, dtype=torch.int32, device="cuda")
+        starts, lens, left = out(n + 1), out(n), out(1)
+        tb.block_tables(ints(held), ints(added), torch.arange(20000, dtype=torch.int32, device="cuda"), ints([left_in]), 16, table, slots,
+                        starts, lens, left)
+        return starts, left
+
+    # a large batch first: its sums are what shared memory is left with
+    call([40] * 1000, [300] * 1000, 20000, out(300000), 30)
+    assert tb.error_flags() == 0
+    slots = out(cap, slots_type)
+    starts, left = call([], [], 11, slots, 30)
+    assert tb.error_flags() == 0
+    assert starts.tolist() == [0] and left.tolist() == [11] and bool((slots == -1).all())
