@@ -485,7 +485,8 @@ int tadma_b200_matvec_q4(const tadma_tensor* x, const tadma_tensor* codes, const
  * Penalties for repeated tokens, biases and a grammar mask on logits
  * [requests, vocab] (F32 / F16 / BF16; out has the same type and may alias),
  * in fp32, rounded once.  ids (I32 [requests, room]) holds each request's
- * lens[r] tokens, the first prompt_lens[r] of them its prompt:
+ * lens[r] tokens (a negative length counts as 0 and one past the room as the
+ * room; both set the error bit), the first prompt_lens[r] of them its prompt:
  *   x = x > 0 ? x / repetition : x * repetition   for tokens among the ids
  *   x = x - frequency * count - presence           for tokens that occur
  *                                  count > 0 times after the prompt

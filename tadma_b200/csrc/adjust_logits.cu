@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const __grid_con
         if (had == 0) listed[atomicAdd(&n_listed, 1)] = (uint16_t)at;
     };
     if (p.ids) {
-        if (len > p.room) bad = true, len = p.room;
+        if (len < 0 || len > p.room) bad = true, len = len < 0 ? 0 : p.room;
         auto note = [&](int64_t i, int32_t id) {
             bad |= id < -1 || id >= p.vocab;
             const int at = place(id);

@@ -60,3 +60,23 @@ def test_block_tables_of_an_empty_batch(slots_type, strided, cap):
     starts, left = call([], [], 11, slots, 30)
     assert tb.error_flags() == 0
     assert starts.tolist() == [0] and left.tolist() == [11] and bool((slots == -1).all())
+
+
+# ------------------------------------------------------------------ logits --
+
+@pytest.mark.parametrize("room", [4, 7, 8, 9000])
+@pytest.mark.parametrize("at", [8, 9])  # ids on 16-byte boundaries, and off them
+@pytest.mark.parametrize("bad", [[-1, -5], [-4, -1 << 31], [-3, -2]])
+def test_logits_negative_lengths_are_empty(room, at, bad):
+    torch = torch_()
+    store = torch.arange(at + 3 * room + 8, dtype=torch.int32, device="cuda") % 50  # tokens before, between and behind the rows
+    ids = store[at:at + 3 * room].view(3, room)
+    x = torch.ones((3, 50), device="cuda")
+    out = torch.zeros_like(x)
+    two = torch.full((3,), 2.0, device="cuda")
+    tb.adjust_logits(x, ids, ints([room, 0, 0]), ints(bad + [2]), out, repetition=two, presence=two, frequency=two)
+    assert tb.error_flags() & INDEX
+    want = torch.ones_like(x)
+    for t in ids[2, :2].tolist():
+        want[2, t] = 0.5 - 2.0 - 2.0
+    assert torch.equal(out, want)
