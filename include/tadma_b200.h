@@ -476,7 +476,8 @@ int64_t tadma_b200_kv4_attention_uses(const tadma_tensor* q, const tadma_tensor*
  * zeros U8 (data NULL: 8) [n, k / g], g a multiple of 32; bias F16 / BF16 /
  * F32 [n] or data NULL.  x F16 / BF16 [m, k] with unit column stride; out F16
  * / BF16 / F32 [m, n], any strides.  codes rows start on 16-byte boundaries.
- * Sums are fp32.  Any number of rows runs; the weights are read once per 16.
+ * Sums are fp32.  Any number of rows to 524280 runs; the weights are read once
+ * per 16.  k is at most 2^31 - 2^14.
  */
 int tadma_b200_matvec_q4(const tadma_tensor* x, const tadma_tensor* codes, const tadma_tensor* scales,
                          const tadma_tensor* zeros, const tadma_tensor* bias, const tadma_tensor* out, void* stream);
