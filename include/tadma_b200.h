@@ -450,8 +450,9 @@ int tadma_b200_kv4_read(const tadma_tensor* k_codes, const tadma_tensor* k_param
  * h reading cache head h / (heads / kv_heads).  q and out are F16 / BF16
  * [requests, heads, dim] of one type, any strides over requests and heads;
  * table I32 [requests, width] names the pages, lens is I32 [requests].  A
- * request of length 0 gives zeros; a length past the table is cut to it;
- * tokens of a page outside the cache are left out.  At most 8192 requests.
+ * request of length 0 gives zeros; a length past the table (or past 2^31 - 64
+ * tokens) is cut to it and a negative one counts as 0, which sets the error
+ * bit; tokens of a page outside the cache are left out.  At most 8192 requests.
  * The work is cut into equal shares for the GPU whatever the lengths, and
  * shares of one head are joined in a fixed order: results do not depend on
  * timing.  `workspace` holds the shares

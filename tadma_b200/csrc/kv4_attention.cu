@@ -74,6 +74,7 @@ constexpr int WARPS = THREADS / 32;
 constexpr int TILE = 32;            // tokens
 constexpr int ROW_COST = 3;         // of a head's start and end, in tiles
 constexpr int MAX_REQUESTS = 8192;  // two int32 each in shared memory
+constexpr int MAX_LEN = 0x7fffffff - 63;  // tokens of a request: a tile more is still an int
 constexpr int MIN_SHARE = 1;        // tiles of a share, where there are few
 constexpr int JOIN_MID = 8, JOIN_MID_FROM = 8;     // warps that join a head cut into more
 constexpr int JOIN_WIDE = 16, JOIN_WIDE_FROM = 48;  // shares than this
@@ -85,7 +86,8 @@ struct AttnParams {
     const char* q;
     char* out;
     const int32_t *table, *lens;
-    int64_t q_row, q_head, o_row, o_head, table_row, table_col, lens_stride, width, pages;
+    int64_t q_row, q_head, o_row, o_head, table_row, table_col, lens_stride, pages;
+    int32_t room;                              // tokens that a request may have
     int32_t requests, per, kv_heads, tiles_h;  // per: query heads of a cache head, in tiles_h tiles
     int32_t page_size, whole;                  // whole: pages hold whole halves of tiles
     int32_t q_vec, o_vec;                      // 16-byte loads of q, 8-byte stores of out
@@ -226,9 +228,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
         const int at = blockIdx.x / RANKS, part = blockIdx.x % RANKS * WARPS + warp;
         cur.request = at / rows;
         cur.row = at - cur.request * rows;
-        const int64_t room = p.width * p.page_size;
         int len = p.lens[cur.request * p.lens_stride];
-        if (len < 0 || len > room) bad = true, len = len < 0 ? 0 : (int)room;
+        if (len < 0 || len > p.room) bad = true, len = len < 0 ? 0 : p.room;
         cur.len = len;
         cur.tile = (int)((int64_t)part * tiles_of(len) / (RANKS * WARPS));
         n = (int)((int64_t)(part + 1) * tiles_of(len) / (RANKS * WARPS)) - cur.tile;
@@ -237,12 +238,11 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
     } else {
         {  // units before each request
             const int each = (p.requests + THREADS - 1) / THREADS, r0 = min(tid * each, p.requests), r1 = min(r0 + each, p.requests);
-            const int64_t room = p.width * p.page_size;
             int64_t sum = 0;
             for (int r = r0; r < r1; r++) {
                 int len = p.lens[r * p.lens_stride];
-                bad |= len < 0 || len > room;
-                len = len < 0 ? 0 : len > room ? (int)room : len;
+                bad |= len < 0 || len > p.room;
+                len = len < 0 ? 0 : len > p.room ? p.room : len;
                 lens[r] = len;
                 sum += units_of(len);
             }
@@ -1006,7 +1006,8 @@ extern "C" int tadma_b200_kv4_attention(const tadma_tensor* q, const tadma_tenso
     p.table_row = table->strides[0];
     p.table_col = table->strides[1];
     p.lens_stride = lens->strides[0];
-    p.width = d.pages > 0 ? table->dims[1] : 0;  // an empty cache holds no token
+    const int64_t room = d.pages > 0 ? table->dims[1] * d.page : 0;  // an empty cache holds no token
+    p.room = room < MAX_LEN ? (int32_t)room : MAX_LEN;
     p.pages = d.pages;
     p.requests = (int32_t)n;
     p.per = (int32_t)per;

@@ -80,3 +80,25 @@ def test_logits_negative_lengths_are_empty(room, at, bad):
     for t in ids[2, :2].tolist():
         want[2, t] = 0.5 - 2.0 - 2.0
     assert torch.equal(out, want)
+
+
+# --------------------------------------------------------------- attention --
+
+def test_attention_of_more_tokens_than_an_int_counts():
+    # One page of 2^20 tokens, 2048 times in a table: a length of 2^31 - 1 is cut to 2^31 - 64 and flagged.  The result
+    # is that of the page alone, but for the rounding of long sums: a warp has at least 2^31 / (148 * 16) tokens, which
+    # at two additions a 32 tokens, each within 2^-23 of the sum, are 56,680 of them: 2^-7.2 of the weighted magnitude
+    # at the very most, and the weights' own sum half of that.
+    torch = torch_()
+    g = gen(11)
+    page, dim = 1 << 20, 64
+    codes = torch.randint(0, 256, (1, 1, page, dim // 2), dtype=torch.uint8, device="cuda", generator=g)
+    params = torch.tensor([0.25, -1.5], device="cuda").half().expand(1, 1, page, 1, 2).contiguous()
+    q = torch.randn((1, 1, dim), device="cuda", generator=g).half()
+    table = torch.zeros((1, 2048), dtype=torch.int32, device="cuda")
+    one, all_ = torch.full_like(q, 7.0), torch.full_like(q, 7.0)
+    tb.kv4_attention(q, codes, params, codes, params, table, ints([page]), 0.125, one)
+    assert tb.error_flags() == 0
+    tb.kv4_attention(q, codes, params, codes, params, table, ints([2 ** 31 - 1]), 0.125, all_)
+    assert tb.error_flags() & INDEX
+    assert float((one.float() - all_.float()).abs().max()) <= 2.0 ** -6 * 2.25 + 2.0 ** -10  # |values| are at most 2.25
