@@ -10,15 +10,16 @@
 // values, query heads in the 8 columns (one query token a request has no 128
 // rows to give a tcgen05 tile).  Codes become fp16 by or-ing them into the
 // mantissa of a power of two (1024 + c in the low nibble of a byte, 64 + c in
-// the high one: exact, one instruction a pair); scale, minimum and that base
-// come in per token and group:
+// the high one) and brought down to c - 8 by an addition, both exact, one
+// instruction a pair each; scale and minimum come in per token and group:
 //
-//   q . k = sum_g s_g (q . (base + c) - base . q) + m_g sum_g q
+//   q . k = sum_g s_g q . (c - 8) + (m_g + 8 s_g) sum_g q
 //   o_d   = sum_t (p_t s_t) (c_td - 8) + sum_t p_t (m_t + 8 s_t)
 //
-// The second sum runs over all tokens and its terms have both signs, so there
-// the base is first brought down to -8 (exact too): with 128 left in, 65,000
-// tokens of mean zero came out 0.7 % off, the sum of the bases cancelling.
+// The additions are what 24-bit sums need: a base left in and taken off the
+// sum cancels, and takes its bits with it.  Scores formed over 1024 + c and
+// 64 + c moved results by up to 1e-3 for queries with a mean, and values over
+// 128 + c by 0.7 % for 65,000 tokens of mean zero.
 //
 // Ranges: q is scaled per head by a power of two to a maximum of 1 to 2, so
 // bf16's exponents fit and its 8 bits stay exact down to 2^-14 of the maximum
@@ -138,6 +139,11 @@ __device__ __forceinline__ uint32_t half2_add(uint32_t x, uint32_t y) {
     return d;
 }
 
+// c - 8 of the codes in the low nibbles of a word's bytes 0 and 2, and of
+// those in the high ones: 1024 + c - 1032 and 64 + c - 72.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w, uint32_t base) { return half2_add(and_or(w, 0x000f000fu, base), 0xe408e408u); }
+__device__ __forceinline__ uint32_t high_codes(uint32_t w, uint32_t base) { return half2_add(and_or(w, 0x00f000f0u, base), 0xd480d480u); }
+
 // d = a b + c, 16 x 8 in fp32 from 16 x 16 and 16 x 8 in fp16.
 __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, const float* c) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
@@ -213,7 +219,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
     using S = Stage<DIM, NG>;
     constexpr int STAGES = S::COUNT;
     extern __shared__ __align__(16) char ring[];
-    int* first = reinterpret_cast<int*>(ring + WARPS * (STAGES * S::BYTES + J * 512 + NG * 64));  // [requests + 1]
+    int* first = reinterpret_cast<int*>(ring + WARPS * (STAGES * S::BYTES + J * 512 + NG * 32));  // [requests + 1]
     int* lens = first + p.requests + 1;                                     // [requests]
     __shared__ int64_t warp_sum[WARPS];
     __shared__ float2 own_ml[WARPS + 1][HEADS];  // with clusters: (maximum, sum) of the warps, then of the CTA
@@ -389,8 +395,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
     // ---- the computing side
     // The query heads' side of the score product: 4 words a lane for each word of codes.
     uint4* const q = reinterpret_cast<uint4*>(ring + WARPS * STAGES * S::BYTES) + warp * J * 32 + lane;
-    // And of heads 2c and 2c + 1 per group the sums of q (x, y) and minus those with the bases (z, w).
-    float4* const q_sums = reinterpret_cast<float4*>(ring + WARPS * (STAGES * S::BYTES + J * 512)) + warp * NG * 4 + c;
+    // And of heads 2c and 2c + 1 per group the sums of q.
+    float2* const q_sums = reinterpret_cast<float2*>(ring + WARPS * (STAGES * S::BYTES + J * 512)) + warp * NG * 4 + c;
     float scale[2], top[2], shift[2], cut[2], sum[2], rest[NG][2], o[J][2][4];
     float v_scale, v_most;               // power of two on the values' scales, and the scale it is good for
     auto start = [&](const Cursor& x) {
@@ -424,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
         const int e = (int)(__float_as_uint(most) >> 23);  // biased
         const float by = __uint_as_float((uint32_t)(e < 1 || e > 253 ? 127 : 254 - e) << 23);
         const float signed_by = p.scale < 0.0f ? -by : by;
-        float part[NG] = {}, base[NG] = {};
+        float part[NG] = {};
 #pragma unroll
         for (int j = 0; j < J; j++) {
             float f[8];
@@ -434,7 +440,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
                 w[j][i] = half_pair(f[2 * i] * signed_by, f[2 * i + 1] * signed_by);
                 const float2 t = from_half_pair(w[j][i]);
                 part[j / JG] += t.x + t.y;
-                base[j / JG] -= 1024.0f * t.x + 64.0f * t.y;
             }
         }
         if constexpr (JG > 1) {
@@ -459,13 +464,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
 #pragma unroll
         for (int i = 0; i < NG; i++) {
 #pragma unroll
-            for (int y = 1; y < 4; y <<= 1) {
-                part[i] += __shfl_xor_sync(0xffffffffu, part[i], y);
-                base[i] += __shfl_xor_sync(0xffffffffu, base[i], y);
-            }
+            for (int y = 1; y < 4; y <<= 1) part[i] += __shfl_xor_sync(0xffffffffu, part[i], y);
             const int of0 = 8 * c, of1 = 8 * c + 4;  // lanes with heads 2c and 2c + 1
-            const float4 sums = make_float4(__shfl_sync(0xffffffffu, part[i], of0), __shfl_sync(0xffffffffu, part[i], of1),
-                                            __shfl_sync(0xffffffffu, base[i], of0), __shfl_sync(0xffffffffu, base[i], of1));
+            const float2 sums = make_float2(__shfl_sync(0xffffffffu, part[i], of0), __shfl_sync(0xffffffffu, part[i], of1));
             if (g == 0) q_sums[4 * i] = sums;
             rest[i][0] = rest[i][1] = 0.0f;
         }
@@ -504,8 +505,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
             }
 #pragma unroll
             for (int i = 0; i < NG; i++) {
-                const float4 qs = q_sums[4 * i];
-                float acc[4] = {qs.z, qs.w, qs.z, qs.w};
+                const float2 qs = q_sums[4 * i];
+                float acc[4] = {};
 #pragma unroll
                 for (int jj = 0; jj < JG; jj++) {
                     uint32_t w[2];
@@ -522,8 +523,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
                     const uint4 qw = q[32 * at];
 #pragma unroll
                     for (int m = 0; m < 2; m++) {
-                        const uint32_t f[4] = {and_or(w[0], 0x000f000fu, p.base_lo), and_or(w[1], 0x000f000fu, p.base_lo),
-                                               and_or(w[0], 0x00f000f0u, p.base_hi), and_or(w[1], 0x00f000f0u, p.base_hi)};
+                        const uint32_t f[4] = {low_codes(w[0], p.base_lo), low_codes(w[1], p.base_lo),
+                                               high_codes(w[0], p.base_hi), high_codes(w[1], p.base_hi)};
                         mma16816(acc, f, m ? qw.z : qw.x, m ? qw.w : qw.y, acc);
                         w[0] >>= 8, w[1] >>= 8;
                     }
@@ -531,8 +532,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     const float2 sm = from_half_pair(kp[r][i]);
-                    s[2 * b + r][0] = fmaf(sm.x, acc[2 * r], fmaf(sm.y, qs.x, s[2 * b + r][0]));
-                    s[2 * b + r][1] = fmaf(sm.x, acc[2 * r + 1], fmaf(sm.y, qs.y, s[2 * b + r][1]));
+                    const float m = fmaf(8.0f, sm.x, sm.y);
+                    s[2 * b + r][0] = fmaf(sm.x, acc[2 * r], fmaf(m, qs.x, s[2 * b + r][0]));
+                    s[2 * b + r][1] = fmaf(sm.x, acc[2 * r + 1], fmaf(m, qs.y, s[2 * b + r][1]));
                 }
             }
         }
@@ -624,11 +626,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
                     uint32_t x0 = __byte_perm(v[0][j / 2], v[1][j / 2], sel), x1 = __byte_perm(v[2][j / 2], v[3][j / 2], sel);
 #pragma unroll
                     for (int m = 0; m < 2; m++) {
-                        // c - 8: 1024 + c - 1032 and 64 + c - 72
-                        const uint32_t f[4] = {half2_add(and_or(x0, 0x000f000fu, p.base_lo), 0xe408e408u),
-                                               half2_add(and_or(x0, 0x00f000f0u, p.base_hi), 0xd480d480u),
-                                               half2_add(and_or(x1, 0x000f000fu, p.base_lo), 0xe408e408u),
-                                               half2_add(and_or(x1, 0x00f000f0u, p.base_hi), 0xd480d480u)};
+                        const uint32_t f[4] = {low_codes(x0, p.base_lo), high_codes(x0, p.base_hi),
+                                               low_codes(x1, p.base_lo), high_codes(x1, p.base_hi)};
                         mma16816(o[j][m], f, hi[0], hi[1], o[j][m]);
                         if constexpr (!PACK) mma16816(o[j][m], f, lo[0], lo[1], o[j][m]);
                         x0 >>= 8, x1 >>= 8;
@@ -886,7 +885,7 @@ bool by_clusters(int64_t requests, int64_t width, const Kv4Dims& d, const Plan& 
 template <typename T, int DIM, int NG, bool PACK, bool CLUSTER>
 int launch_attention(const AttnParams& p, cudaStream_t s) {
     const size_t lists = CLUSTER ? 0 : (2 * (size_t)p.requests + 1) * sizeof(int);
-    const size_t smem = WARPS * (Stage<DIM, NG>::COUNT * Stage<DIM, NG>::BYTES + DIM / 32 * 512 + NG * 64) + lists;
+    const size_t smem = WARPS * (Stage<DIM, NG>::COUNT * Stage<DIM, NG>::BYTES + DIM / 32 * 512 + NG * 32) + lists;
     auto* kernel = kv4_attention_kernel<T, DIM, NG, PACK, CLUSTER>;
     // The ring decides how many CTAs an SM holds: all of its shared memory, once per device and kernel.
     static std::atomic<uint64_t> set{0};

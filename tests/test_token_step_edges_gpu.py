@@ -102,3 +102,51 @@ def test_attention_of_more_tokens_than_an_int_counts():
     tb.kv4_attention(q, codes, params, codes, params, table, ints([2 ** 31 - 1]), 0.125, all_)
     assert tb.error_flags() & INDEX
     assert float((one.float() - all_.float()).abs().max()) <= 2.0 ** -6 * 2.25 + 2.0 ** -10  # |values| are at most 2.25
+
+
+def cache_rows(codes, params, slots):
+    """Host rows [tokens, heads, ...] of a cache at those slots."""
+    page = codes.shape[2]
+    return [t.cpu().numpy()[slots // page, :, slots % page] for t in (codes, params)]
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim,group", [(64, 32), (64, 64), (128, 64), (128, 128), (256, 32), (256, 256)])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (8, 1)])
+@pytest.mark.parametrize("spare", [0, 3000])
+def test_attention_scores_of_queries_with_a_mean(dtype, dim, group, heads, kv_heads, spare):
+    # Keys (c - 8) s with c = 8 but in 8 of their places, queries of about 4 everywhere: what the scores are made of is
+    # small beside any multiple of sum q.  A step of mma.sync adds 17 terms, aligned to the largest and cut to 24 bits or
+    # more: 17 * 2^-24 < 2^-19.9 of the largest, which is at most A = sum |q||k|.  So a score errs by less than
+    # (dim / 16 + 4) 2^-19.9 A scale, a weight by twice the largest of these and 2^-17 for the exponential and the two
+    # halves of p s, and the values' sum by as much a step again: two steps (with the halves apart) a 16 tokens.
+    torch = torch_()
+    g = gen(dim + group + heads)
+    lens, page, scale = [300, 77], 16, 0.25
+    params, codes = [], []
+    for i in range(2):
+        s = 2.0 ** torch.randint(-1, 2, (26, kv_heads, page, dim // group, 1), device="cuda", generator=g)
+        params.append(torch.cat([s, -8 * s], -1).half())
+        nibbles = torch.full((26, kv_heads, page, dim), 8, dtype=torch.uint8, device="cuda")
+        at = torch.rand(nibbles.shape, device="cuda", generator=g).argsort(-1)[..., :8]
+        nibbles.scatter_(-1, at, torch.randint(7, 10, at.shape, dtype=torch.uint8, device="cuda", generator=g))
+        if i == 1:
+            nibbles = torch.randint(0, 16, nibbles.shape, dtype=torch.uint8, device="cuda", generator=g)
+        codes.append(nibbles[..., 0::2] | nibbles[..., 1::2] << 4)
+    table = torch.randperm(26, device="cuda", generator=g).int()[None].repeat(2, 1)
+    table = torch.cat([table, torch.full((2, spare), -1, dtype=torch.int32, device="cuda")], 1)
+    q = (4 + 0.5 * torch.randn((2, heads, dim), device="cuda", generator=g)).clamp(min=1).to(getattr(torch, dtype))
+    out = torch.full_like(q, 7.0)
+    tb.kv4_attention(q, codes[0], params[0], codes[1], params[1], table, ints(lens), scale, out)
+    assert tb.error_flags() == 0
+    got, qh, tab = f64(out), f64(q), table.cpu().numpy()
+    for r, n in enumerate(lens):
+        t = np.arange(n)
+        slots = tab[r][t // page].astype(np.int64) * page + t % page
+        kk, vv = (ref.values(*cache_rows(c, p, slots)) for c, p in zip(codes, params))
+        want, mass, top = ref.attention(qh[r], kk, vv, scale)
+        step = 17 * 2.0 ** -24
+        weight = 2 * (dim / 16 + 4) * step * top[:, None] + 2.0 ** -17
+        tol = UNIT[dtype] * np.abs(want) + (weight + (n / 8 + 4) * step) * (mass + np.abs(want))
+        off = np.abs(got[r] - want)
+        assert np.all(off <= tol), (r, float((off / tol).max()), float(off.max()))
