@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
     // And of heads 2c and 2c + 1 per group the sums of q.
     float2* const q_sums = reinterpret_cast<float2*>(ring + WARPS * (STAGES * S::BYTES + J * 512)) + warp * NG * 4 + c;
     float scale[2], top[2], shift[2], cut[2], sum[2], rest[NG][2], o[J][2][4];
-    float v_scale, v_most;               // power of two on the values' scales, and the scale it is good for
+    float v_scale, v_most;               // power of two on the values' scales, and the largest that it is good for
     auto start = [&](const Cursor& x) {
         const int head = p.tiles_h == 1 ? x.row : x.row / p.tiles_h, h0 = (x.row - head * p.tiles_h) * HEADS;
         const int of = h0 + (PACK ? g & 3 : g);  // the query head of this lane's column
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
         }
         __syncwarp();
         v_scale = 1.0f;
-        v_most = -1.0f;
+        v_most = 0.0f;  // the first scale above 0 decides
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
@@ -560,13 +560,16 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
         for (int u = 0; u < 4; u++)
 #pragma unroll
             for (int i = 0; i < NG; i++) met = fmaxf(met, fabsf(from_half_pair(vp[u][i]).x));
-        if (__any_sync(0xffffffffu, t[0] > cut[0] || t[1] > cut[1] || met > v_most)) {
+        // The values' power of two brings the largest scale that was met to 32..64, and changes again for a tile whose
+        // scales are larger, or all below 2^-12 of what it is good for: weights of 1 keep 2^-18 of themselves.
+        constexpr float FEW = 4096.0f;
+        if (__any_sync(0xffffffffu, t[0] > cut[0] || t[1] > cut[1] || met > v_most) || __all_sync(0xffffffffu, met * FEW < v_most)) {
             float by = 1.0f;
 #pragma unroll
             for (int y = 4; y < 32; y <<= 1) met = fmaxf(met, __shfl_xor_sync(0xffffffffu, met, y));
-            if (met > v_most) {
+            if (met > v_most || (met > 0.0f && met * FEW < v_most)) {
                 const int e = (int)(__float_as_uint(met) >> 23);  // biased, 103 and up for an fp16
-                const float now = e < 1 ? 1.0f : __uint_as_float((uint32_t)(254 + 5 - e) << 23);
+                const float now = __uint_as_float((uint32_t)(254 + 5 - e) << 23);
                 by = now / v_scale;
                 v_scale = now;
                 v_most = 64.0f / now;

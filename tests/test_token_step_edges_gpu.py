@@ -150,3 +150,45 @@ def test_attention_scores_of_queries_with_a_mean(dtype, dim, group, heads, kv_he
         tol = UNIT[dtype] * np.abs(want) + (weight + (n / 8 + 4) * step) * (mass + np.abs(want))
         off = np.abs(got[r] - want)
         assert np.all(off <= tol), (r, float((off / tol).max()), float(off.max()))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (8, 1)])
+@pytest.mark.parametrize("requests,n", [(1, 4096), (200, 352)])
+@pytest.mark.parametrize("first,ahead,rest", [(0.0, 8.0, 1e-3), (64.0, -40.0, 2.0 ** -20), (2.0 ** -20, -40.0, 64.0)])
+@pytest.mark.parametrize("spread", [False, True])  # scores that differ from token to token
+def test_attention_of_value_scales_far_apart(heads, kv_heads, requests, n, first, ahead, rest, spread):
+    # Every fourth tile of 32 tokens has value scales of another size and scores `ahead` of the others', so that a
+    # running scaling of the weights has to follow.  Products p s keep 2^-18 of themselves and sums some 2^-20 a step
+    # (n / 8 steps at most), well inside 2^-9; results are rounded to bfloat16.
+    torch = torch_()
+    g = gen(requests + heads)
+    dim, page = 64, 16
+    pages = requests * n // page
+    tiles = (torch.arange(n, device="cuda") // 32 % 4 == 0).view(1, n // page, 1, page)
+
+    def per_token(there, elsewhere):
+        t = torch.where(tiles, float(there), float(elsewhere)).expand(requests, n // page, kv_heads, page)
+        return t.reshape(pages, kv_heads, page, 1)
+
+    zero = torch.zeros((pages, kv_heads, page, 1), device="cuda")
+    k = [torch.zeros((pages, kv_heads, page, dim // 2), dtype=torch.uint8, device="cuda"),
+         torch.stack([zero, per_token(ahead / 8, 0)], -1).half()]
+    if spread:
+        k[0].random_(0, 256, generator=g)
+        k[1][..., 0] = 0.125
+    v = [torch.randint(0, 4, (pages, kv_heads, page, dim), dtype=torch.uint8, device="cuda", generator=g) + 12,
+         torch.stack([per_token(first, rest), zero], -1).half()]
+    v[0] = v[0][..., 0::2] | v[0][..., 1::2] << 4
+    q = torch.ones((requests, heads, dim), dtype=torch.bfloat16, device="cuda")
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").view(requests, -1)
+    out = torch.full_like(q, 7.0)
+    tb.kv4_attention(q, *k, *v, table, ints([n] * requests), 0.125, out)  # scores are 8 times the keys' value
+    assert tb.error_flags() == 0
+    got = f64(out)
+    for r in range(0, requests, 7):
+        slots = np.arange(r * n, (r + 1) * n)
+        kk, vv = (ref.values(*cache_rows(*c, slots)) for c in (k, v))
+        want, mass, _ = ref.attention(np.ones((heads, dim)), kk, vv, 0.125)
+        off = np.abs(got[r] - want)
+        tol = UNIT["bfloat16"] * np.abs(want) + 2.0 ** -9 * mass
+        assert np.all(off <= tol), (r, float((off / tol).max()))
