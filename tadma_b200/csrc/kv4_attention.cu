@@ -470,11 +470,12 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
             if (g == 0) q_sums[4 * i] = sums;
             rest[i][0] = rest[i][1] = 0.0f;
         }
-        // A scale of 0 gives equal weights: any tiny scale does, and keeps -inf out of a product with 0.
-        const float s = fabsf(p.scale) > 1e-30f ? fabsf(p.scale) : 1e-30f;
+        // Scores of a query brought to 1..2 are below 2^30 (256 values of at most 16 * 65504 each), so any factor below
+        // 2^-120 gives equal weights, as 0 does; 2^-120 keeps -inf out of a product with 0.
+        const float s = fabsf(p.scale) * LOG2E;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            scale[h] = __shfl_sync(0xffffffffu, s * LOG2E / by, 4 * (2 * c + h));
+            scale[h] = __shfl_sync(0xffffffffu, fmaxf(s / by, 0x1p-120f), 4 * (2 * c + h));
             top[h] = cut[h] = -INFINITY;
             shift[h] = sum[h] = 0.0f;
         }

@@ -192,3 +192,34 @@ def test_attention_of_value_scales_far_apart(heads, kv_heads, requests, n, first
         off = np.abs(got[r] - want)
         tol = UNIT["bfloat16"] * np.abs(want) + 2.0 ** -9 * mass
         assert np.all(off <= tol), (r, float((off / tol).max()))
+
+
+@pytest.mark.parametrize("size,scale", [(2.0 ** -100, 0.0), (2.0 ** -60, 0.0), (1.0, 0.0), (2.0 ** 110, 0.0), (2.0 ** -110, 1e-12), (2.0 ** -90, -1e-20),
+                                        (2.0 ** -100, 2.0 ** 97), (2.0 ** 100, -(2.0 ** -103))])
+@pytest.mark.parametrize("spare", [0, 3000])
+def test_attention_of_tiny_and_huge_queries(size, scale, spare):
+    # bfloat16 queries of any magnitude.  A score errs by 2^-16 of sum |q||k| scale and a weight by 2^-13, as bounded for
+    # ordinary queries; sizes are powers of two.
+    torch = torch_()
+    g = gen(21)
+    lens, heads, dim, page = [77, 40, 1], 4, 64, 16
+    pages = 12
+    caches = []
+    for _ in range(2):
+        s = torch.rand((pages, 2, page, 2, 1), device="cuda", generator=g) * 0.3 + 0.1
+        caches.append((torch.randint(0, 256, (pages, 2, page, dim // 2), dtype=torch.uint8, device="cuda", generator=g),
+                       torch.cat([s, -7.5 * s], -1).half()))
+    table = torch.cat([torch.arange(15, device="cuda").view(3, 5).int() % pages, torch.full((3, spare), -1, dtype=torch.int32, device="cuda")], 1)
+    q = (torch.randn((3, heads, dim), device="cuda", generator=g).bfloat16().double() * size).bfloat16()
+    out = torch.full_like(q, 7.0)
+    tb.kv4_attention(q, *caches[0], *caches[1], table, ints(lens), scale, out)
+    assert tb.error_flags() == 0
+    got, tab = f64(out), table.cpu().numpy()
+    for r, n in enumerate(lens):
+        t = np.arange(n)
+        slots = tab[r][t // page].astype(np.int64) * page + t % page
+        kk, vv = (ref.values(*cache_rows(*c, slots)) for c in caches)
+        want, mass, top = ref.attention(f64(q)[r], kk, vv, scale)
+        tol = UNIT["bfloat16"] * np.abs(want) + (2.0 ** -13 + 2.0 ** -16 * top[:, None]) * (mass + np.abs(want))
+        off = np.abs(got[r] - want)
+        assert np.all(off <= tol), (r, float(np.nanmax(off / tol)))
