@@ -374,7 +374,8 @@ int launch_shape(MatvecParams& p, int cluster, cudaStream_t s) {
     const int rows = p.m < S::ROWS ? (int)p.m : S::ROWS;
     const int bytes = S::bytes(rows);
     p.cluster = cluster;
-    if (bytes > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    // Always the most that the shape takes: calls of other threads with fewer rows may not lower it before this launch.
+    if (bytes > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(S::ROWS));
     if (e != cudaSuccess) return cuda_fail(e, "tadma_b200_matvec_q4 shared memory");
     const dim3 grid((unsigned)((p.n + S::COLS - 1) / S::COLS * cluster), (unsigned)((p.m + S::ROWS - 1) / S::ROWS));
     (void)launch_pdl_cluster(kernel, grid, cluster, dim3(32 * S::WARPS), bytes, s, p);

@@ -223,3 +223,47 @@ def test_attention_of_tiny_and_huge_queries(size, scale, spare):
         tol = UNIT["bfloat16"] * np.abs(want) + (2.0 ** -13 + 2.0 ** -16 * top[:, None]) * (mass + np.abs(want))
         off = np.abs(got[r] - want)
         assert np.all(off <= tol), (r, float(np.nanmax(off / tol)))
+
+
+# ----------------------------------------------------------------- threads --
+
+def in_threads(*calls, times=4000):
+    """Runs the calls `times` times each, every one in a thread and on a stream of its own; raises what one raises."""
+    import threading
+    torch = torch_()
+    errors, gate = [], threading.Barrier(len(calls))
+
+    def work(call, stream):
+        gate.wait()
+        try:
+            for _ in range(times):
+                call(stream)
+        except Exception as e:  # noqa: BLE001  (handed to the test)
+            errors.append(e)
+
+    streams = [torch.cuda.Stream() for _ in calls]
+    threads = [threading.Thread(target=work, args=(c, s.cuda_stream)) for c, s in zip(calls, streams)]
+    torch.cuda.synchronize()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    if errors:
+        raise errors[0]
+
+
+def test_matvec_of_few_and_more_rows_in_two_threads():
+    # One kernel, 51,200 bytes of shared memory a CTA for 2 rows and 100,352 for 8.
+    torch = torch_()
+    g = gen(31)
+    n, k = 256, 512
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=g)
+    scales = torch.full((n, k // 128), 0.01, dtype=torch.float16, device="cuda")
+    xs = [torch.randn((m, k), device="cuda", generator=g).half() for m in (2, 8)]
+    outs = [torch.zeros((x.shape[0], n), dtype=torch.float32, device="cuda") for x in xs]
+    in_threads(*[lambda stream, x=x, out=out: tb.matvec_q4(x, codes, scales, out, stream=stream) for x, out in zip(xs, outs)])
+    for x, out in zip(xs, outs):
+        alone = torch.zeros_like(out)
+        tb.matvec_q4(x, codes, scales, alone)
+        assert torch.equal(out, alone)
