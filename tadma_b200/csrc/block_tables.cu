@@ -197,7 +197,9 @@ extern "C" int tadma_b200_block_tables(const tadma_tensor* held, const tadma_ten
     p.page = page_size;
     const size_t smem = (3 * (size_t)n + 2) * sizeof(int);
     cudaError_t e = cudaSuccess;
-    if (smem > 48 * 1024) e = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // Always the most that a call takes: one of another thread with fewer requests may not lower it before this launch.
+    constexpr int MOST = (3 * MAX_REQUESTS + 2) * sizeof(int);
+    if (smem > 48 * 1024) e = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST);
     if (e != cudaSuccess) return cuda_fail(e, "tadma_b200_block_tables shared memory");
     // A token a thread; one CTA for a small batch's single tokens.
     const int64_t want = (p.cap + THREADS - 1) / THREADS, most = 4 * sm_count();

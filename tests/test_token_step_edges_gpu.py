@@ -267,3 +267,22 @@ def test_matvec_of_few_and_more_rows_in_two_threads():
         alone = torch.zeros_like(out)
         tb.matvec_q4(x, codes, scales, alone)
         assert torch.equal(out, alone)
+
+
+def test_block_tables_of_many_and_more_requests_in_two_threads():
+    # 12 bytes of shared memory a request: 60,008 for 5000 and 192,008 for 16000.
+    torch = torch_()
+
+    def make(n):
+        held, added = ints([17] * n), ints([1] * n)
+        table = torch.zeros((n, 2), dtype=torch.int32, device="cuda")
+        out = [torch.full((k,), 99, dtype=torch.int32, device="cuda") for k in (n, n + 1, n, 1)]
+        args = [held, added, ints([0]), ints([1]), 16, table, *out]
+        return lambda stream: tb.block_tables(*args, stream=stream), out
+
+    (few, few_out), (more, more_out) = make(5000), make(16000)
+    in_threads(few, more)
+    assert tb.error_flags() == 0
+    for n, (slots, starts, lens, left) in ((5000, few_out), (16000, more_out)):
+        assert bool((slots == 1).all()) and torch.equal(starts, torch.arange(n + 1, dtype=torch.int32, device="cuda"))
+        assert bool((lens == 18).all()) and left.tolist() == [1]
