@@ -411,7 +411,9 @@ int tadma_b200_gather(const tadma_tensor* table, int32_t axis, const tadma_tenso
  *   lens[r]     = held[r] + added[r]
  *   slots[t]    = table[r, p / page_size] * page_size + p % page_size for
  *                 token t of request r, p = held[r] + t - starts[r]; -1 where
- *                 the table has no page, and past the last token (I64 / I32)
+ *                 the table has no page, and past the last token (I64 / I32);
+ *                 -1 and the error bit where p is past the table's width, or
+ *                 I32 cannot hold the slot
  *   left[0]     = num_free[0] - sum of need: pages left in the pool, negative
  *                 by as many as were missing
  * table is I32 [requests, width]; at most 16384 requests.  The outputs may

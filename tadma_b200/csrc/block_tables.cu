@@ -135,10 +135,13 @@ __global__ void __launch_bounds__(THREADS) block_tables_kernel(const __grid_cons
             if (e < p.width) {
                 const int page = e < mine ? p.table[r * p.table_row + e * p.table_col] : page_of(firsts[r] + (e - mine));
                 if (page >= 0) slot = (int64_t)page * p.page + (pos - e * p.page);
+                if (!p.slots64 && slot > 0x7fffffff) bad = true, slot = -1;
+            } else {
+                bad = true;  // in the last held page, which the table has no room for, or in a new one
             }
         }
         if (p.slots64) reinterpret_cast<int64_t*>(p.slots)[t * p.slots_stride] = slot;
-        else reinterpret_cast<int32_t*>(p.slots)[t * p.slots_stride] = slot > 0x7fffffff ? -1 : (int32_t)slot;
+        else reinterpret_cast<int32_t*>(p.slots)[t * p.slots_stride] = (int32_t)slot;
     }
     if (bad) atomicOr(&g_error_word, 1u << TADMA_ERR_INDEX);
 }

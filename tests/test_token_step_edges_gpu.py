@@ -62,6 +62,30 @@ def test_block_tables_of_an_empty_batch(slots_type, strided, cap):
     assert starts.tolist() == [0] and left.tolist() == [11] and bool((slots == -1).all())
 
 
+def one_request(held, added, page_size, entries, slots_type="int64"):
+    """(slots, flags) of one request with that table row and an empty pool."""
+    torch = torch_()
+    slots, starts, lens, left = (torch.full((k,), 99, dtype=getattr(torch, t), device="cuda")
+                                 for k, t in ((added, slots_type), (2, "int32"), (1, "int32"), (1, "int32")))
+    tb.block_tables(ints([held]), ints([added]), ints([0]), ints([0]), page_size, ints([entries]), slots, starts, lens, left)
+    return slots.tolist(), tb.error_flags()
+
+
+def test_block_tables_flags_slots_that_int32_cannot_hold():
+    page_size = 1 << 20
+    at = 2 ** 31 - 2  # of page 2047 the last place but one
+    assert one_request(at % page_size, 2, page_size, [2047], "int32") == ([at, at + 1], 0)
+    assert one_request(5, 2, page_size, [2048], "int64") == ([2 ** 31 + 5, 2 ** 31 + 6], 0)
+    assert one_request(5, 2, page_size, [2048], "int32") == ([-1, -1], INDEX)
+
+
+def test_block_tables_flags_tokens_past_the_width():
+    # the last held page is half full, so no new page is needed, but the table has no entry for it
+    assert one_request(20, 3, 16, [4]) == ([-1] * 3, INDEX)
+    assert one_request(20, 3, 16, [4, 7]) == ([116, 117, 118], 0)
+    assert one_request(20, 3, 16, [4, -1]) == ([-1] * 3, 0)  # an entry without a page is the caller's
+
+
 # ------------------------------------------------------------------ logits --
 
 @pytest.mark.parametrize("room", [4, 7, 8, 9000])
