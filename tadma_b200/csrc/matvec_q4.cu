@@ -14,7 +14,9 @@
 //   s (sum x (16 + c) - (16 + z) sum x)
 //
 // which loses no more than 2 bits against summing c - z, and saves a
-// subtraction for every pair of codes.
+// subtraction for every pair of codes.  It needs 8 bits of range above the
+// result's, and an infinity among x makes it a difference of two: a result that
+// is not finite is summed again as the formula stands, one thread a result.
 //
 // The warps of a cluster's CTAs take turns at blocks of KB k of the same
 // RT * 16 columns: each has a ring of stages of its own, filled by cp.async,
@@ -105,6 +107,24 @@ struct Pair<__nv_bfloat16> {
                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 };
+
+// out[row, col] before its bias as the formula stands, for results that are not finite in the fast form.
+template <typename T>
+__device__ __noinline__ float plain_sum(const MatvecParams& p, int64_t row, int col) {
+    float v = 0.0f;
+    for (int k = 0; k < (int)p.k && !isnan(v); k += 32) {  // a group is a multiple of 32
+        const int64_t at = p.groups.div32((uint32_t)k);
+        const float s = load_as<float>(p.scales, p.s_dtype, col * p.s_row + at * p.s_col), z = p.zeros ? (float)p.zeros[col * p.z_row + at * p.z_col] : 8.0f;
+        const uint4 codes = *reinterpret_cast<const uint4*>(p.codes + col * p.c_row + k / 2);
+        const T* const x = reinterpret_cast<const T*>(p.x) + row * p.x_row + k;
+        const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+        float part = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; i++) part = fmaf((float)x[i], ((float)(w[i / 8] >> (4 * (i % 8)) & 15) - z) * s, part);
+        v += part;
+    }
+    return v;
+}
 
 // cp.async of 16 bytes, or 16 zeros where there is nothing to read.
 __device__ __forceinline__ void cp_async16_or_zero(void* smem, const void* gmem, bool there) {
@@ -341,6 +361,7 @@ __global__ void __launch_bounds__(32 * Shape<RT, NT, SUB>::WARPS, RT == 4 && NT 
     auto finish = [&](int e, float v) {
         const int col = e % S::COLS, row = e / S::COLS;
         if (n0 + col < own || n0 + col >= p.n) return;
+        if (!isfinite(v)) v = plain_sum<T>(p, m0 + row, n0 + col);
         if (p.bias) v += load_as<float>(p.bias, p.b_dtype, (int64_t)(n0 + col) * p.b_stride);
         store_from(p.out, p.o_dtype, (m0 + row) * p.o_row + (int64_t)(n0 + col) * p.o_col, v);
     };

@@ -249,6 +249,44 @@ def test_attention_of_tiny_and_huge_queries(size, scale, spare):
         assert np.all(off <= tol), (r, float(np.nanmax(off / tol)))
 
 
+# ------------------------------------------------------------------ matvec --
+
+@pytest.mark.parametrize("dtype,size", [("float16", 1.0), ("bfloat16", 1.0), ("bfloat16", 2.0 ** 118), ("bfloat16", 2.0 ** 125)])
+@pytest.mark.parametrize("m", [1, 5, 12])
+@pytest.mark.parametrize("n,k,group,zeros", [(5, 64, 32, True), (100, 640, 64, False), (300, 8192, 128, True), (6000, 2112, 32, True)])
+def test_matvec_of_infinite_and_huge_rows(dtype, size, m, n, k, group, zeros):
+    # Row 0 has an infinity, row 1 two of them, row 2 a NaN; the others are numbers, of the end of bfloat16's range
+    # (scales keep the results inside fp32's).  A result is an infinity or NaN where the formula gives one; numbers err by a
+    # rounding a term of 32, one a block of 32, and that of the fast form, 2^-18 of sum |x| 16 s.
+    torch = torch_()
+    g = gen(m + n + k)
+    x = (torch.randn((m, k), device="cuda", generator=g).clamp(-4, 4) * size).to(getattr(torch, dtype))
+    x[0, k // 3] = float("inf")
+    if m > 2:
+        x[1, 7], x[1, k - 1] = float("-inf"), float("inf")
+        x[2, k // 2] = float("nan")
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=g)
+    scales = ((torch.rand((n, k // group), device="cuda", generator=g) + 0.5) * 2.0 ** -13).to(getattr(torch, dtype))
+    z = torch.randint(0, 16, (n, k // group), dtype=torch.uint8, device="cuda", generator=g) if zeros else None
+    bias = torch.randn(n, device="cuda", generator=g)
+    out = torch.full((m, n), 7.0, device="cuda")
+    tb.matvec_q4(x, codes, scales, out, zeros=z, bias=bias)
+    w = ref.weights(codes.cpu().numpy(), f64(scales), None if z is None else z.cpu().numpy())
+    xh, got = f64(x), f64(out)
+    plain = np.where(np.isfinite(xh), xh, 0.0)
+    want, size_of = plain @ w.T + f64(bias), np.abs(plain) @ np.abs(w).T
+    fast = np.abs(plain) @ np.repeat(16 * f64(scales), group, 1).T
+    with np.errstate(invalid="ignore"):
+        for r in range(min(m, 3)):
+            for at in np.flatnonzero(~np.isfinite(xh[r])):
+                want[r] += xh[r, at] * w[:, at]
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(np.isposinf(got), np.isposinf(want)) and np.array_equal(np.isneginf(got), np.isneginf(want))
+    finite = np.isfinite(want)
+    tol = UNIT["float32"] * np.abs(want) + (33 + k / 32) * 2.0 ** -24 * size_of + 2.0 ** -18 * fast
+    assert np.all(np.abs(got - want)[finite] <= tol[finite])
+
+
 # ----------------------------------------------------------------- threads --
 
 def in_threads(*calls, times=4000):
