@@ -427,7 +427,9 @@ int tadma_b200_block_tables(const tadma_tensor* held, const tadma_tensor* added,
 /*
  * Writes tokens into the cache: k and v (F16 / BF16, [tokens, kv_heads, dim],
  * any strides over tokens and heads) go to slots[t] (I64 / I32); a slot
- * of -1 is skipped, two equal slots leave either token.  Per group
+ * of -1 is skipped.  The slots of a call are distinct, as block_tables' are:
+ * what a slot holds that different tokens name is not defined (codes of one,
+ * parameters of another); no other slot changes.  Per group
  *   minimum = f16(min x), scale = f16((max x - min x) / 15),
  *   code    = round-half-even((x - minimum) / scale) clamped to 0..15
  * (0 for scale 0).  A group with a value that is not finite, or whose scale

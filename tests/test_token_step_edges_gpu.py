@@ -86,6 +86,36 @@ def test_block_tables_flags_tokens_past_the_width():
     assert one_request(20, 3, 16, [4, -1]) == ([-1] * 3, 0)  # an entry without a page is the caller's
 
 
+# -------------------------------------------------------------- the cache --
+
+@pytest.mark.parametrize("dim,group", [(64, 32), (128, 128), (256, 64)])
+def test_append_of_equal_slots_changes_no_other(dim, group):
+    # 600 tokens on 40 slots.  Where all tokens of a slot are the same it holds them; what the others hold is not defined.
+    torch = torch_()
+    g = gen(dim)
+    tokens, heads, page = 600, 2, 16
+    slots = torch.arange(tokens, device="cuda") % 40 + 17
+    x = [torch.randn((tokens, heads, dim), device="cuda", generator=g).half() for _ in range(2)]
+    same = slots % 2 == 0
+    for t in x:
+        t[same] = t[slots[same] - 17]
+    shape = (8, heads, page)
+    caches = [(torch.randint(0, 256, shape + (dim // 2,), dtype=torch.uint8, device="cuda", generator=g),
+               torch.randn(shape + (dim // group, 2), device="cuda", generator=g).half()) for _ in range(2)]
+    before = [[t.clone() for t in c] for c in caches]
+    tb.kv4_append(*x, slots, *caches[0], *caches[1])
+    assert tb.error_flags() == 0
+    others = np.setdiff1d(np.arange(8 * page), slots.cpu().numpy())
+    even = slots[same].unique().cpu().numpy()
+    for i in range(2):
+        for now, was in zip(cache_rows(*caches[i], others), cache_rows(*before[i], others)):
+            assert np.array_equal(now, was)
+        alone = [torch.zeros_like(t) for t in caches[i]]
+        tb.kv4_append(x[i][:40], x[i][:40], slots[:40], *alone, *alone)
+        for now, want in zip(cache_rows(*caches[i], even), cache_rows(*alone, even)):
+            assert np.array_equal(now, want)
+
+
 # ------------------------------------------------------------------ logits --
 
 @pytest.mark.parametrize("room", [4, 7, 8, 9000])
