@@ -22,10 +22,6 @@
 
 namespace tadma_b200 {
 
-static __device__ unsigned int g_error_word;
-
-cudaError_t adjust_logits_error_word(uint32_t* flags, bool clear) { return read_error_word(g_error_word, flags, clear); }
-
 namespace {
 
 // A token's word: whether the prompt has it, 1 + its last entry among
@@ -42,6 +38,7 @@ struct LogitsParams {
     const float *rep, *pres, *freq, *bias;
     int64_t ids_row, ids_col, room, prompt_stride, lens_stride, rep_stride, pres_stride, freq_stride;
     int64_t bid_row, bid_col, bias_row, bias_col, n_bias, mask_row, mask_col;
+    uint32_t* errors;
 };
 
 // The logit of token v with the word c.
@@ -175,7 +172,7 @@ __global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const __grid_con
         } while (had != saw);
         if (bias_entry(saw) < entry) list(at, saw);
     }
-    if (bad) atomicOr(&g_error_word, 1u << TADMA_ERR_INDEX);
+    if (bad) atomicOr(p.errors, 1u << TADMA_ERR_INDEX);
     __syncthreads();
     if (n_listed == 0) return;
 
@@ -302,6 +299,8 @@ extern "C" int tadma_b200_adjust_logits(const tadma_tensor* logits, const tadma_
         p.mask_row = mask->strides[0];
         p.mask_col = mask->strides[1];
     }
+    const cudaError_t e = error_word(&p.errors);
+    if (e != cudaSuccess) return cuda_fail(e, "tadma_b200_adjust_logits error word");
     cudaStream_t s = (cudaStream_t)stream;
     switch (logits->dtype) {
     case TADMA_F32: return launch_logits<float>(p, b, s);

@@ -15,10 +15,6 @@
 
 namespace tadma_b200 {
 
-static __device__ unsigned int g_error_word;
-
-cudaError_t block_tables_error_word(uint32_t* flags, bool clear) { return read_error_word(g_error_word, flags, clear); }
-
 namespace {
 
 constexpr int THREADS = 512;
@@ -31,6 +27,7 @@ struct TablesParams {
     char* slots;
     int64_t slots_stride, cap;
     int32_t slots64, n, page;
+    uint32_t* errors;
 };
 
 __device__ __forceinline__ int count_at(const IntVec& v, int64_t i) {
@@ -143,7 +140,7 @@ __global__ void __launch_bounds__(THREADS) block_tables_kernel(const __grid_cons
         if (p.slots64) reinterpret_cast<int64_t*>(p.slots)[t * p.slots_stride] = slot;
         else reinterpret_cast<int32_t*>(p.slots)[t * p.slots_stride] = (int32_t)slot;
     }
-    if (bad) atomicOr(&g_error_word, 1u << TADMA_ERR_INDEX);
+    if (bad) atomicOr(p.errors, 1u << TADMA_ERR_INDEX);
 }
 
 }  // namespace
@@ -199,7 +196,8 @@ extern "C" int tadma_b200_block_tables(const tadma_tensor* held, const tadma_ten
     p.n = (int)n;
     p.page = page_size;
     const size_t smem = (3 * (size_t)n + 2) * sizeof(int);
-    cudaError_t e = cudaSuccess;
+    cudaError_t e = error_word(&p.errors);
+    if (e != cudaSuccess) return cuda_fail(e, "tadma_b200_block_tables error word");
     // Always the most that a call takes: one of another thread with fewer requests may not lower it before this launch.
     constexpr int MOST = (3 * MAX_REQUESTS + 2) * sizeof(int);
     if (smem > 48 * 1024) e = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST);

@@ -20,6 +20,7 @@
 // writes its output once and reads each gathered row once, so at config 5
 // sizes it is an HBM-bound copy.
 // Any other layout takes a per-element path with the same semantics.
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 #include <unordered_map>
@@ -30,9 +31,21 @@
 
 namespace tadma_b200 {
 
-// Per-device error word of the gather kernels (bit 1 << TADMA_ERR_INDEX = an
-// id was out of range).
+// Per-device error word of the gather and token-step kernels (bit 1 <<
+// TADMA_ERR_INDEX = an id, slot, page or length was out of range).
 static __device__ unsigned int g_error_word;
+
+cudaError_t error_word(uint32_t** word) {
+    static std::atomic<uint32_t*> known[64];  // by device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    *word = dev < 64 ? known[dev].load() : nullptr;
+    if (*word) return cudaSuccess;
+    e = cudaGetSymbolAddress(reinterpret_cast<void**>(word), g_error_word);
+    if (e == cudaSuccess && dev < 64) known[dev].store(*word);
+    return e;
+}
 
 namespace {
 
@@ -401,11 +414,6 @@ extern "C" int tadma_b200_error_flags(uint32_t* flags, int32_t clear) {
         unsigned int z = 0;
         e = cudaMemcpyToSymbol(g_error_word, &z, sizeof(z));
         if (e != cudaSuccess) return cuda_fail(e, "tadma_b200_error_flags clear");
-    }
-    // The token-step kernels keep words of their own.
-    for (auto part : {block_tables_error_word, kv4_error_word, kv4_attention_error_word, adjust_logits_error_word}) {
-        e = part(flags, clear != 0);
-        if (e != cudaSuccess) return cuda_fail(e, "tadma_b200_error_flags token step");
     }
     return TADMA_OK;
 }

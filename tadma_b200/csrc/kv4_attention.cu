@@ -64,10 +64,6 @@
 
 namespace tadma_b200 {
 
-static __device__ unsigned int g_error_word;
-
-cudaError_t kv4_attention_error_word(uint32_t* flags, bool clear) { return read_error_word(g_error_word, flags, clear); }
-
 namespace {
 
 constexpr int THREADS = 128;
@@ -101,6 +97,7 @@ struct AttnParams {
     uint32_t base_lo, base_hi;                 // 1024 and 64, twice
     DivMod page;
     float scale;
+    uint32_t* errors;
     // workspace
     int32_t* first;  // [requests + 1] units before a request (one head)
     float2* ml;      // [2 * shares][heads of a tile] (maximum, sum)
@@ -271,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
             if (blockIdx.x == 0)
                 for (int r = tid; r <= p.requests; r += THREADS) p.first[r] = first[r];
         }
-        if (bad) atomicOr(&g_error_word, 1u << TADMA_ERR_INDEX);
+        if (bad) atomicOr(p.errors, 1u << TADMA_ERR_INDEX);
         bad = false;
 
         const Shares shares(p, first[p.requests]);
@@ -775,7 +772,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(DIM, NG)) kv4_attention_k
         }
         cluster.sync();  // nobody leaves while its part is read
     }
-    if (bad) atomicOr(&g_error_word, 1u << TADMA_ERR_INDEX);
+    if (bad) atomicOr(p.errors, 1u << TADMA_ERR_INDEX);
 }
 
 // Joins the shares of the rows that were cut, and writes zeros for requests
@@ -1042,6 +1039,8 @@ extern "C" int tadma_b200_kv4_attention(const tadma_tensor* q, const tadma_tenso
     p.shares = plan.shares;
     p.page = DivMod((uint64_t)d.page);
     p.scale = (float)scale;
+    const cudaError_t ew = error_word(&p.errors);
+    if (ew != cudaSuccess) return cuda_fail(ew, "tadma_b200_kv4_attention error word");
     cudaStream_t s = (cudaStream_t)stream;
     p.clusters = by_clusters(n, table->dims[1], d, plan);
     if (p.clusters) return q->dtype == TADMA_F16 ? launch_dim<__half>(p, d, s) : launch_dim<__nv_bfloat16>(p, d, s);

@@ -30,10 +30,6 @@
 
 namespace tadma_b200 {
 
-static __device__ unsigned int g_error_word;
-
-cudaError_t kv4_error_word(uint32_t* flags, bool clear) { return read_error_word(g_error_word, flags, clear); }
-
 int check_kv4(const tadma_tensor* codes, const tadma_tensor* params, const char* name, bool first, Kv4Dims& d,
               Kv4View& v) {
     const std::string n = name;
@@ -100,6 +96,7 @@ struct CacheParams {
     uint32_t two23;  // 2^23 as a float: a parameter, for (w & mask) | two23 to be one instruction
     int64_t rows;    // tokens * heads
     DivMod page, headm;
+    uint32_t* errors;
 };
 
 constexpr int LANES = 8;  // of a row
@@ -124,7 +121,7 @@ struct Place {
                                        : (int64_t) reinterpret_cast<const int32_t*>(p.slots)[tok * p.slots_stride];
         held = slot >= 0 && slot < p.pages * (int64_t)p.page.d;
         if (!held) {
-            if (slot != -1) atomicOr(&g_error_word, 1u << TADMA_ERR_INDEX);
+            if (slot != -1) atomicOr(p.errors, 1u << TADMA_ERR_INDEX);
             return;
         }
         page = p.wide ? (uint32_t)p.page.div((uint64_t)slot) : p.page.div32((uint32_t)slot);
@@ -427,11 +424,13 @@ int cache_params(const tadma_tensor* k, const tadma_tensor* v, const char* kn, c
     return TADMA_OK;
 }
 
-int launch_cache(void (*kernel)(CacheParams), const CacheParams& p, void* stream, const char* what) {
+int launch_cache(void (*kernel)(CacheParams), CacheParams p, void* stream, const char* what) {
     const int64_t grid = (p.rows * LANES + THREADS - 1) / THREADS;
     if (grid > 0x7fffffff) return fail(TADMA_ERR_UNSUPPORTED, std::string(what) + ": too many tokens for one call");
+    cudaError_t e = error_word(&p.errors);
+    if (e != cudaSuccess) return cuda_fail(e, what);
     (void)launch_pdl(kernel, dim3((unsigned)grid), dim3(THREADS), 0, (cudaStream_t)stream, p);
-    const cudaError_t e = cudaGetLastError();
+    e = cudaGetLastError();
     return e == cudaSuccess ? TADMA_OK : cuda_fail(e, what);
 }
 

@@ -1,29 +1,15 @@
-// token_step.cuh - what the token-step kernels share: the error word of a
-// translation unit and its host access, and the checks of cache descriptors.
+// token_step.cuh - what the token-step kernels share: the error word, cluster
+// launches, and the checks of cache descriptors.
 #pragma once
 
 #include "common.cuh"
 
 namespace tadma_b200 {
 
-// ORs the unit's error word into *flags (when given) and clears it on request.
-cudaError_t block_tables_error_word(uint32_t* flags, bool clear);
-cudaError_t kv4_error_word(uint32_t* flags, bool clear);
-cudaError_t kv4_attention_error_word(uint32_t* flags, bool clear);
-cudaError_t adjust_logits_error_word(uint32_t* flags, bool clear);
-
-template <typename Word>
-cudaError_t read_error_word(const Word& symbol, uint32_t* flags, bool clear) {
-    unsigned int w = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(&w, symbol, sizeof(w));
-    if (e != cudaSuccess) return e;
-    if (flags) *flags |= w;
-    if (clear && w) {
-        const unsigned int z = 0;
-        e = cudaMemcpyToSymbol(symbol, &z, sizeof(z));
-    }
-    return e;
-}
+// The address of the error word on the current device: gather.cu has it, and
+// the kernels of other units take it as a parameter, so that
+// tadma_b200_error_flags has one word to copy.
+cudaError_t error_word(uint32_t** word);
 
 // launch_pdl with clusters of `cluster` CTAs along the grid's x.
 template <typename... KArgs, typename... Args>

@@ -378,3 +378,64 @@ def test_block_tables_of_many_and_more_requests_in_two_threads():
     for n, (slots, starts, lens, left) in ((5000, few_out), (16000, more_out)):
         assert bool((slots == 1).all()) and torch.equal(starts, torch.arange(n + 1, dtype=torch.int32, device="cuda"))
         assert bool((lens == 18).all()) and left.tolist() == [1]
+
+
+# -------------------------------------------------------------- error word --
+
+def test_error_flags_copies_one_word():
+    # whatever operator set it: reading is one copy from the device, clearing one to it
+    torch = torch_()
+    x = torch.ones((1, 8), device="cuda")
+    tb.gather(x, 0, ints([0]), torch.empty_like(x))
+    tb.error_flags()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU, torch.profiler.ProfilerActivity.CUDA]) as prof:
+        assert tb.error_flags(clear=False) == 0
+        assert tb.error_flags(clear=True) == 0
+    copies = [e.name for e in prof.events() if e.name.startswith("Memcpy")]
+    assert sorted(c.split()[1] for c in copies) == ["DtoH", "DtoH", "HtoD"], copies
+
+
+def test_error_word_is_one_for_all_operators():
+    torch = torch_()
+    x = torch.ones((1, 8), device="cuda")
+    cache = [torch.zeros((1, 1, 16, 32), dtype=torch.uint8, device="cuda"), torch.zeros((1, 1, 16, 1, 2), dtype=torch.float16, device="cuda")]
+    rows = torch.zeros((1, 1, 64), dtype=torch.float16, device="cuda")
+    spare = [ints([0] * n) for n in (2, 1, 1)]
+    wrong = {"gather": lambda: tb.gather(x, 0, ints([5]), torch.empty_like(x)),
+             "block_tables": lambda: tb.block_tables(ints([0]), ints([1]), ints([0]), ints([0]), 16, ints([[0]]), ints([0]), *spare),
+             "kv4_append": lambda: tb.kv4_append(rows, rows, ints([16]), *cache, *cache),
+             "kv4_read": lambda: tb.kv4_read(*cache, *cache, ints([-2]), rows.clone(), rows.clone()),
+             "kv4_attention": lambda: tb.kv4_attention(rows, *cache, *cache, ints([[0]]), ints([17]), 0.125, rows.clone()),
+             "adjust_logits": lambda: tb.adjust_logits(x, ints([[8]]), ints([0]), ints([1]), torch.empty_like(x))}
+    for name, call in wrong.items():
+        assert tb.error_flags() == 0, name
+        call()
+        assert tb.error_flags(clear=False) == INDEX, name
+        assert tb.error_flags() == INDEX, name
+
+
+def test_first_call_may_be_captured():
+    # a process whose first calls of the library are recorded into a graph
+    import os
+    import subprocess
+    import sys
+    program = """
+import torch, tadma_b200 as tb
+i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+x, out, ids, one = torch.ones((1, 8), device="cuda"), torch.zeros((1, 8), device="cuda"), i([[3, 9]]), i([2])
+cache = [torch.zeros((1, 1, 16, 32), dtype=torch.uint8, device="cuda"), torch.zeros((1, 1, 16, 1, 2), dtype=torch.float16, device="cuda")]
+rows, zero, pen = torch.zeros((1, 1, 64), dtype=torch.float16, device="cuda"), i([0]), torch.ones(1, device="cuda")
+got, lens, table = rows.clone() + 1, i([1]), i([[0]])
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    tb.kv4_append(rows, rows, zero, *cache, *cache)
+    tb.kv4_attention(rows, *cache, *cache, table, lens, 0.125, got)
+    tb.adjust_logits(x, ids, zero, one, out, presence=pen)
+g.replay()
+torch.cuda.synchronize()
+assert out.tolist() == [[1, 1, 1, 0, 1, 1, 1, 1]] and bool((got == 0).all()) and tb.error_flags() == 16
+print("replayed")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", program], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "replayed" in r.stdout, r.stdout + r.stderr
