@@ -345,23 +345,77 @@ def prepare_adjust_logits(logits, ids, prompt_lens, lens, out, repetition=None, 
 # One-shot calls of a token step are bound by the host, so they go through the
 # extension module _pycall (csrc/pycall.c) instead of ctypes.
 
-_calls = None        # the module, once loaded
+def _operand(t):
+    if t is None or isinstance(t, TadmaTensor):
+        return t
+    if not hasattr(t, "data_ptr"):
+        raise TypeError("expected a tensor or a tensor descriptor")
+    d = TadmaTensor(data=t.data_ptr(), dtype=int(_TORCH_DT.get(t.dtype, -1)), rank=t.dim())  # the call refuses what it does not know
+    for i, (n, s) in enumerate(zip(t.shape[:MAX_RANK], t.stride())):
+        d.dims[i], d.strides[i] = n, s
+    return d
+
+
+class _CtypesCalls:
+    """What _pycall offers, through ctypes (10 to 45 us more host time a call): for a Python whose headers the build did
+    not have."""
+
+    @staticmethod
+    def _refs(tensors):
+        return [None if t is None else ctypes.byref(t) for t in map(_operand, tensors)]
+
+    def _call(self, name, tensors, stream):
+        return getattr(lib(), "tadma_b200_" + name)(*self._refs(tensors), stream)
+
+    def block_tables(self, *a):
+        r = self._refs(a[:9])
+        page = a[9] if 0 <= a[9] <= 0x7fffffff else 0
+        return lib().tadma_b200_block_tables(*r[:4], page, *r[4:], a[10])
+
+    def kv4_append(self, *a):
+        return self._call("kv4_append", a[:7], a[7])
+
+    def kv4_read(self, *a):
+        return self._call("kv4_read", a[:7], a[7])
+
+    def kv4_attention(self, *a):
+        r = self._refs(a[:8])
+        scale, ws, n, stream, alloc = a[8:]
+        made = None
+        if not ws and alloc is not None:
+            n = lib().tadma_b200_kv4_attention_uses(r[0], r[1], r[2], r[5])
+            if n > 0:
+                made = alloc(n)
+                ws = made.data_ptr()
+        return lib().tadma_b200_kv4_attention(*r[:7], scale, r[7], ws, n, stream)
+
+    def matvec_q4(self, *a):
+        return self._call("matvec_q4", a[:6], a[6])
+
+    def adjust_logits(self, *a):
+        return self._call("adjust_logits", a[:11], a[11])
+
+
+_calls = None        # the module (or what stands in for it), once loaded
 _stream_now = None   # address of torch's current stream
 
 
 def _load_steps():
     global _calls, _stream_now
     lib()  # its error where the library has not been built; and the module finds it loaded
-    from . import _pycall
     torch = _torch()
     torch_dtype_code(torch.empty(0))
-    _pycall.set_dtypes({t: int(c) for t, c in _TORCH_DT.items()})
+    try:
+        from . import _pycall as calls
+        calls.set_dtypes({t: int(c) for t, c in _TORCH_DT.items()})
+    except ImportError:
+        calls = _CtypesCalls()
     raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), torch.cuda.current_device
     if raw is None:
         _stream_now = lambda: torch.cuda.current_stream().cuda_stream  # noqa: E731
     else:
         _stream_now = lambda: raw(device())  # noqa: E731  (without the object, which takes 3 us)
-    _calls = _pycall
+    _calls = calls
     return _calls
 
 
