@@ -12,7 +12,7 @@
 // less than the logits themselves up to some 8000 ids; calls with room for
 // more take slices of 16384.
 //
-// 256 requests of 50257 fp32 logits with 2000 ids and 64 biases each take 26.2
+// 256 requests of 50257 fp32 logits with 2000 ids and 64 biases each take 25.9
 // us on the device (4.0 TB/s; 17 us without ids and biases: the chain lengths -
 // ids - counts - listed tokens bounds it), one request with 300 ids 3.7 us.
 #include <cmath>

@@ -27,7 +27,8 @@
 // warp, raised and lowered with the scales met, and goes into the product as
 // the sum of two fp16 (22 bits), the second in columns of its own; where a
 // cache head has at most 4 query heads the upper 4 columns are free for it.
-// All sums are fp32.
+// All sums are fp32; those of mma.sync are cut and not rounded, which over
+// 65,000 tokens leaves some 2^-17 of a result.
 //
 // Tiles travel through a ring of stages in shared memory, one per warp, so
 // there is no barrier wider than a warp: cp.async fills the stages ahead while
@@ -43,18 +44,21 @@
 // with 8 heads, 9 shares a head: 66.2 us, 65.9 with 8 warps), with 8 where
 // heads have more than 8 shares (8 requests of 65001 tokens: 160.5 us, 167.2
 // with one, 163.0 with 16), with 16 from 48 (one request of 32000 tokens: 21.4
-// us, 23.5 with 8, 71.7 with one; dim 128).
+// us, 23.5 with 8, 71.7 with one; dim 128; times of the kernel before its
+// scores were formed over c - 8, which moved all of them by a percent or less).
 //
 // Where all heads together are few and their pages too, a cluster of 8 CTAs
 // takes one head instead, its 32 warps equal parts of the tokens, and joins
 // them over distributed shared memory: one launch, no workspace (one request
-// of 1000 tokens, 16 heads of dim 64: 5.9 us on the device, 11.8 by shares).
+// of 1000 tokens, 16 heads of dim 64: 5.8 us on the device, 11.8 by shares).
 //
 // 8 requests of 65001 tokens (64 query and 8 cache heads of dim 128, groups of
-// 64) take 159 us on the device, 3.7 TB/s of codes and parameters; 128 requests
-// of 0 to 8191 tokens (32 and 8 heads, groups of 128) 48.5 us.  Instructions
-// bound both: some 800 a tile, of which a warp finishes one in 2.2 us beside
-// the 11 others of its SM.
+// 64) take 161 us on the device, 3.6 TB/s of codes and parameters; 128 requests
+// of 0 to 8191 tokens (32 and 8 heads, groups of 128) 50.4 us.  No unit of the
+// GPU is full: in the first the issue slots are 64 % taken (845 instructions a
+// tile), DRAM 42 %, the tensor pipe 29 %.  A tile is one dependent chain -
+// copies, scores, exponentials, weights, values - of 2.2 us, and registers
+// (163 a thread) and the ring leave 12 warps an SM to run beside each other.
 #include <cooperative_groups.h>
 
 #include <atomic>

@@ -20,10 +20,12 @@
 // again (exact) and multiplied by the scale over its place's power of 16.
 //
 // Appending 8191 tokens of 8 heads, dim 128, groups of 32, fp16, and reading
-// them back takes 26.3 us on the device (17.6 and 9.7 us each by itself), 3.4
-// TB/s of rows and codes: the instructions bound it (721 a warp that appends,
-// 774 without packed fp32 pairs).  48 tokens take 5.9 us for the two, all
-// latency.
+// them back takes 26.2 us on the device (17.6 and 9.7 us each by itself), 3.4
+// TB/s of rows and codes.  Of the time to append, 10 us are its instructions
+// (721 a warp, 774 without packed fp32 pairs; issue slots 65 % taken), the rest
+// is waiting: a warp lives for 4 rows, and slot, page and values are fetched one
+// after the other with nothing of another row in flight.  48 tokens take 5.9 us
+// for the two, all latency.
 #include <type_traits>
 
 #include "token_step.cuh"

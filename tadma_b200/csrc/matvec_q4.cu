@@ -13,10 +13,12 @@
 //
 //   s (sum x (16 + c) - (16 + z) sum x)
 //
-// which loses no more than 2 bits against summing c - z, and saves a
-// subtraction for every pair of codes.  It needs 8 bits of range above the
-// result's, and an infinity among x makes it a difference of two: a result that
-// is not finite is summed again as the formula stands, one thread a result.
+// which saves a subtraction for every pair of codes.  Against summing c - z it
+// loses nothing for x of mean zero (8192 k: 2e-7 of the results' size, as fp32
+// does) and up to 5 bits for x with a mean (8e-6 against 3e-7), as mma.sync cuts
+// its sums and the cuts add up.  It needs 8 bits of range above the result's,
+// and an infinity among x makes it a difference of two: a result that is not
+// finite is summed again as the formula stands, one thread a result.
 //
 // The warps of a cluster's CTAs take turns at blocks of KB k of the same
 // RT * 16 columns: each has a ring of stages of its own, filled by cp.async,
@@ -25,10 +27,14 @@
 // the L1 that CTAs of an SM share).  Where the lanes of a load would meet in a
 // bank, rows are padded or every other row has its halves exchanged.
 //
-// 8192 x 8192 with one row takes 14.1 us on the device (2.5 TB/s), 50257 x 4096
-// with 8 rows, groups of 64 and zero points 44.3 us (2.6 TB/s), 768 x 768 with
-// one row 2.6 us.  A warp's instructions bound the large ones (46 for 16 x 32
-// codes with groups of 64, 39.5 with 128), its launch the small.
+// 8192 x 8192 with one row takes 13.5 us on the device (2.5 TB/s), 50257 x 4096
+// with 8 rows, groups of 64 and zero points 44.2 us (2.6 TB/s), 768 x 768 with
+// one row 2.6 us, its launch.  In the large ones no unit of the GPU is full: the
+// vocabulary's has its issue slots 49 % taken (46 instructions for 16 x 32 codes
+// with groups of 64, 39.5 with 128), DRAM 29 %, the tensor pipe 19 %.  A warp's
+// decode, products and scaling are one dependent chain with at most four warps a
+// scheduler; the first has only 4 turns of a ring between its start and the
+// cluster's join, the second 786 CTAs on 592 places.
 #include <cooperative_groups.h>
 
 #include <type_traits>
