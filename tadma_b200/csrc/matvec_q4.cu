@@ -507,7 +507,7 @@ extern "C" int tadma_b200_matvec_q4(const tadma_tensor* x, const tadma_tensor* c
     if (k > 0 && ((uintptr_t)codes->data % 16 != 0 || (n > 1 && codes->strides[0] % 16 != 0)))
         return fail(TADMA_ERR_UNSUPPORTED, "codes rows must start on 16-byte boundaries");
     // Counters of k are int and run up to two turns of a cluster's rings (2 x 4096 k) past the end.
-    if (k > 0x7fffffff - 16384 || n > 0x7fffff00 || m > (int64_t)65535 * 8) return fail(TADMA_ERR_UNSUPPORTED, "matvec_q4: too large");
+    if (k > (1ll << 31) - 16384 || n > 0x7fffff00 || m > (int64_t)65535 * 8) return fail(TADMA_ERR_UNSUPPORTED, "matvec_q4: too large");
     if (m == 0 || n == 0) return TADMA_OK;
 
     MatvecParams p{};
